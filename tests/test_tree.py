@@ -1,0 +1,27 @@
+"""CPU tests of the tree itself: what its tools may do on a GPU, and what the build entry point does."""
+import os, re
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+SKIP_DIRS = {'.git', '.pytest_cache', '__pycache__', '_work', 'gpurun_out', 'profiles', 'build', 'build_tmp', '_ref', 'golden'}
+SOURCE = ('.hip', '.hpp', '.h', '.c', '.cc', '.cpp', '.s', '.py', '.sh', '.mk', '.txt')
+
+def sources(sub='.'):
+    """(path from the root, text) of the sources, scripts and build files below sub"""
+    for base, dirs, files in os.walk(os.path.join(ROOT, sub)):
+        dirs[:] = [d for d in dirs if d not in SKIP_DIRS]
+        for f in sorted(files):
+            p = os.path.join(base, f)
+            if (f.endswith(SOURCE) or f == 'Makefile') and not os.path.samefile(p, __file__):
+                yield os.path.relpath(p, ROOT), open(p, encoding='utf-8', errors='replace').read()
+
+def test_no_tool_brings_a_hang_about():
+    """a launch that does not end is looked for by reading the code and on the CPU: no tool repeats a workload until one stops or holds the device's queues beside it"""
+    bad = [p for p, t in sources('tools') if re.search(r'hang\d*\b|repro loop|holds? .{0,12}hardware queues', p + '\n' + t, re.I)]
+    assert not bad, bad
+
+def test_the_number_of_hardware_queues_is_a_fixed_small_one():
+    for p, t in sources():
+        for m in re.finditer(r"GPU_MAX_HW_QUEUES['\"]?\]?\s*[,=]\s*([^,);\s]+)", t):
+            v = m.group(1).strip('\'"')
+            assert v.isdigit() and int(v) <= 16, (p, m.group(0))
