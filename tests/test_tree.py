@@ -25,3 +25,9 @@ def test_the_number_of_hardware_queues_is_a_fixed_small_one():
         for m in re.finditer(r"GPU_MAX_HW_QUEUES['\"]?\]?\s*[,=]\s*([^,);\s]+)", t):
             v = m.group(1).strip('\'"')
             assert v.isdigit() and int(v) <= 16, (p, m.group(0))
+
+def test_no_gpu_code_writes_through_the_scalar_cache():
+    """scalar stores and atomics, and that cache's write-back and discard, are named in no source, comments included: what a kernel writes goes through vector stores"""
+    op = re.compile(r'(?<![A-Za-z0-9])s_(?:(?:buffer|scratch)_)?(?:store|atomic)_|(?<![A-Za-z0-9])s_dcache_(?:wb|discard)')
+    bad = ['%s:%d' % (p, t.count('\n', 0, m.start()) + 1) for p, t in sources() for m in op.finditer(t)]
+    assert not bad, bad
