@@ -31,3 +31,28 @@ def test_no_gpu_code_writes_through_the_scalar_cache():
     op = re.compile(r'(?<![A-Za-z0-9])s_(?:(?:buffer|scratch)_)?(?:store|atomic)_|(?<![A-Za-z0-9])s_dcache_(?:wb|discard)')
     bad = ['%s:%d' % (p, t.count('\n', 0, m.start()) + 1) for p, t in sources() for m in op.finditer(t)]
     assert not bad, bad
+
+@pytest.fixture
+def build_commands(monkeypatch):
+    """build() with its commands recorded instead of run, on a machine where the reference's directory holds the given files (None: no such directory)"""
+    import __graft_entry__ as entry
+    real = {n: getattr(os.path, n) for n in ('exists', 'isfile', 'isdir')}
+    def run(reference):
+        top = '/root/reference'; cmds = []
+        def faked(name):
+            def f(p):
+                s = os.fspath(p).rstrip('/')
+                if s == top: return reference is not None and name != 'isfile'
+                if s.startswith(top + '/'): return name != 'isdir' and s[len(top) + 1:] in (reference or ())
+                return real[name](p)
+            return f
+        for n in real: monkeypatch.setattr(os.path, n, faked(n))
+        monkeypatch.setattr(entry, '_run', lambda cmd, cwd=ROOT: cmds.append(list(cmd)))
+        entry.build()
+        return cmds
+    return run
+
+@pytest.mark.parametrize('reference,built', [(None, False), ((), False), (('README.md',), False), (('minialign.c', 'gaba.c', 'gaba_wrap.h'), True)],
+                         ids=['no-directory', 'empty-directory', 'no-sources', 'sources'])
+def test_the_reference_is_compiled_only_where_its_sources_are(build_commands, reference, built):
+    assert any(c[0] == 'make' and 'ref' in c for c in build_commands(reference)) is built
