@@ -56,3 +56,9 @@ def build_commands(monkeypatch):
                          ids=['no-directory', 'empty-directory', 'no-sources', 'sources'])
 def test_the_reference_is_compiled_only_where_its_sources_are(build_commands, reference, built):
     assert any(c[0] == 'make' and 'ref' in c for c in build_commands(reference)) is built
+
+def test_build_compiles_every_time_it_is_called(build_commands):
+    """build() is the check that the tree builds: a library that is there already does not stand in for its sources"""
+    made = [os.path.relpath(c[c.index('-o') + 1], ROOT) for c in build_commands(None) if '-o' in c]
+    assert {'minialign_amd/libminialign_amd.so', 'minialign_amd/libminialign_amd_prof.so', 'minialign_amd/minialign', 'tools/gensim', 'tools/samcheck'} <= set(made), made
+    assert any(c[0] == 'make' and 'oracle' in c and ('-B' in c or '--always-make' in c) for c in build_commands(None))
