@@ -2,7 +2,7 @@
 # FETCH_SIZE / WRITE_SIZE of rocprofv3 against kernels of known HBM traffic (tools/ubench/traffic_cal.hip), separate --pmc passes, kernel trace only.
 # Usage (GPU box): tools/pmc_calibrate.sh <out.json>
 OUT=${1:-gpurun_out/pmc_calibration.json}; D=$(mktemp -d /tmp/pmccal.XXXX); cd "$(dirname "$0")/.."; R=$PWD; export TMPDIR=/tmp
-[ -x tools/ubench/traffic_cal ] || hipcc --offload-arch=gfx950 -O3 -Wno-unused-value -o tools/ubench/traffic_cal tools/ubench/traffic_cal.hip || exit 1
+[ -x tools/ubench/traffic_cal ] || hipcc --offload-arch=gfx950 -O3 -Wno-unused-value -Xclang -target-feature -Xclang -packed-fp32-ops -o tools/ubench/traffic_cal tools/ubench/traffic_cal.hip || exit 1
 for c in FETCH_SIZE WRITE_SIZE; do
 	( cd /tmp && rocprofv3 --kernel-trace --pmc $c --output-format csv -d $D/$c -o p -- $R/tools/ubench/traffic_cal 8 > $D/$c.log 2>&1 )
 done

@@ -2,7 +2,7 @@
 // instruction gives?  (The step of the DP fill copies the vector that moves with the step; folding the shift into the three readers of the copy would take one VALU
 // instruction out of 33.)  Measured on gfx950: v_add_u32_dpp and v_sub_u32_dpp (dpp(src0) - src1) do; v_subrev_u32_dpp does NOT compute src1 - dpp(src0): it computes
 // dpp(src1) - src0 -- the lane shift lands on the minuend in both forms, so "x - shifted(y)" has no single instruction, the fill needs it once per direction
-// (gfv - shr(dh) going right, df - shl(dv) going down), and the copy stays.   hipcc --offload-arch=gfx950 -O3 -o dpp_vop2 tools/ubench/dpp_vop2.hip && ./dpp_vop2
+// (gfv - shr(dh) going right, df - shl(dv) going down), and the copy stays.   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o dpp_vop2 tools/ubench/dpp_vop2.hip && ./dpp_vop2
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdint>

@@ -3,7 +3,7 @@
  *   pinned     hipMemcpyAsync from a hipHostMalloc'd copy (the ceiling of the link)
  *   register   hipHostRegister of the whole buffer (timed), then hipMemcpyAsync from it, then hipHostUnregister (timed)
  *   staged     T host threads copy 32 MB pieces into a ring of R pinned buffers, hipMemcpyAsync from there (what the library's reader does)
- * usage: h2d_rate [GB = 4]     build: hipcc --offload-arch=gfx950 -O2 -o h2d_rate h2d_rate.hip -lpthread */
+ * usage: h2d_rate [GB = 4]     build: hipcc --offload-arch=gfx950 -O2 -Xclang -target-feature -Xclang -packed-fp32-ops -o h2d_rate h2d_rate.hip -lpthread */
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 #include <stdlib.h>
