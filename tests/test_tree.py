@@ -88,3 +88,8 @@ def test_the_library_holds_no_packed_fp32(tmp_path):
         asm = subprocess.run([objdump, '-d', f], cwd=tmp_path, check=True, stdout=subprocess.PIPE).stdout.decode()
         assert asm.count('\n') > 1000
         assert not re.search(r'\bv_pk_(?:add|mul|fma)_f32\b', asm), f
+
+def test_pinned_memory_is_allocated_pinned():
+    """memory that exists already is not registered with the driver: what has to be pinned is allocated that way (hipHostMalloc)"""
+    bad = [p for p, t in sources() if re.search(r'\b(?:hip|cuda)Host(?:Unr|R)egister\w*\s*\(', t)]
+    assert not bad, bad

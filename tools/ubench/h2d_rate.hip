@@ -1,7 +1,6 @@
 /* h2d_rate.hip -- how fast does text in ordinary (pageable) host memory get into HBM?  The ways the reader could take, timed on one buffer:
  *   pageable   hipMemcpy straight from the buffer (the runtime stages it itself)
  *   pinned     hipMemcpyAsync from a hipHostMalloc'd copy (the ceiling of the link)
- *   register   hipHostRegister of the whole buffer (timed), then hipMemcpyAsync from it, then hipHostUnregister (timed)
  *   staged     T host threads copy 32 MB pieces into a ring of R pinned buffers, hipMemcpyAsync from there (what the library's reader does)
  * usage: h2d_rate [GB = 4]     build: hipcc --offload-arch=gfx950 -O2 -Xclang -target-feature -Xclang -packed-fp32-ops -o h2d_rate h2d_rate.hip -lpthread */
 #include <hip/hip_runtime.h>
@@ -54,19 +53,6 @@ int main(int argc, char **argv)
 		char *pin = nullptr; const size_t pn = n < (2ull << 30) ? n : (2ull << 30); OK(hipHostMalloc(&pin, pn, hipHostMallocDefault)); memcpy(pin, host, pn);
 		for(int rep = 0; rep < 2; rep++) { t0 = now_ms(); OK(hipMemcpyAsync(dev, pin, pn, hipMemcpyHostToDevice, st)); OK(hipStreamSynchronize(st)); printf("pinned source (ceiling)     : %6.1f GB/s\n", pn * 1e-6 / (now_ms() - t0)); }
 		OK(hipHostFree(pin));
-	}
-	for(int rep = 0; rep < 2; rep++) {
-		t0 = now_ms(); hipError_t r = hipHostRegister(host, n, hipHostRegisterDefault); const double t_reg = now_ms() - t0;
-		if(r != hipSuccess) { printf("hipHostRegister failed: %s\n", hipGetErrorString(r)); break; }
-		t0 = now_ms(); OK(hipMemcpyAsync(dev, host, n, hipMemcpyHostToDevice, st)); OK(hipStreamSynchronize(st)); const double t_cp = now_ms() - t0;
-		t0 = now_ms(); OK(hipHostUnregister(host)); const double t_un = now_ms() - t0;
-		printf("register %.0f ms (%5.1f GB/s) + copy %6.1f GB/s + unregister %.0f ms: %6.1f GB/s all told\n", t_reg, n * 1e-6 / t_reg, n * 1e-6 / t_cp, t_un, n * 1e-6 / (t_reg + t_cp + t_un));
-	}
-	/* registering piece by piece just ahead of the copy (what a reader over a mapped file could do) */
-	for(size_t piece : { (size_t)64 << 20, (size_t)256 << 20 }) {
-		t0 = now_ms();
-		for(size_t o = 0; o < n; o += piece) { const size_t nb = n - o < piece ? n - o : piece; OK(hipHostRegister(host + o, nb, hipHostRegisterDefault)); OK(hipMemcpyAsync(dev + o, host + o, nb, hipMemcpyHostToDevice, st)); OK(hipStreamSynchronize(st)); OK(hipHostUnregister(host + o)); }
-		printf("register / copy / unregister in pieces of %3zu MB: %6.1f GB/s\n", piece >> 20, n * 1e-6 / (now_ms() - t0));
 	}
 	for(size_t piece : { (size_t)8 << 20, (size_t)32 << 20, (size_t)64 << 20 }) for(unsigned T : { 1u, 2u, 4u, 8u, 12u, 16u, 24u }) for(int R : { 2, 4 }) {
 		if(R == 2 && T != 8) continue;
