@@ -93,3 +93,8 @@ def test_pinned_memory_is_allocated_pinned():
     """memory that exists already is not registered with the driver: what has to be pinned is allocated that way (hipHostMalloc)"""
     bad = [p for p, t in sources() if re.search(r'\b(?:hip|cuda)Host(?:Unr|R)egister\w*\s*\(', t)]
     assert not bad, bad
+
+def test_the_tools_name_only_tests_that_are_there():
+    have = {m for p, t in sources('tests') for m in re.findall(r'def (test_\w+)', t)} | {os.path.basename(p)[:-3] for p, t in sources('tests') if p.endswith('.py')}
+    gone = ['%s: %s' % (p, m) for p, t in sources('tools') for m in re.findall(r'\btest_\w+', t) if m not in have]
+    assert not gone, gone
